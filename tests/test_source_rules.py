@@ -1,0 +1,29 @@
+"""Rules over the source text that no run shows: each guards against a way of building or driving
+the GPU that has failed without an error of its own (a hang, a fault, a wrong sum now and then)."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _sources(*tops, ext=(".hip", ".h", ".cpp", ".py", ".sh", ".c", "Makefile")):
+    """(path relative to the root, text) of every source file under the given folders or files"""
+    out = []
+    for top in tops:
+        p = os.path.join(ROOT, top)
+        names = [p] if os.path.isfile(p) else [os.path.join(d, f) for d, _, fs in os.walk(p) for f in fs]
+        for n in names:
+            if n.endswith(ext) and os.path.abspath(n) != os.path.abspath(__file__):
+                with open(n, encoding="utf-8") as f:
+                    out.append((os.path.relpath(n, ROOT), f.read()))
+    assert out
+    return out
+
+
+def test_every_stream_has_the_default_priority():
+    """Work on streams of different priorities beside each other can hang the device."""
+    bad = re.compile(r"hipStreamCreateWithPriority|cudaStreamCreateWithPriority|StreamPriorityRange|"
+                     r"is_high_priority_stream|Stream\([^)]*priority")
+    hits = ["%s: %s" % (n, m.group(0)) for n, t in _sources("veneur_amd", "include", "tools", "tests", "bench.py",
+                                                           "__graft_entry__.py") for m in bad.finditer(t)]
+    assert not hits, hits

@@ -93,21 +93,27 @@ void check_slots_host(const uint32_t* slot, uint64_t n, uint32_t cap, const char
 #ifndef VN_REPLAY_EIGHTHS
 #define VN_REPLAY_EIGHTHS 6
 #endif
+// A stream at the default priority: on the mask's CUs (a CU-masked stream gets a hardware queue
+// of its own), or unmasked when the mask is empty.  No stream of the engine has another
+// priority: work on streams of different priorities beside each other can hang the device.
+hipStream_t stream_on(const std::vector<uint32_t>& mask) {
+  hipStream_t s = nullptr;
+  if (mask.empty()) VN_HIP_CHECK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+  else VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&s, (uint32_t)mask.size(), mask.data()));
+  return s;
+}
+
 void create_impl(vn_engine* e) {
   VN_HIP_CHECK(hipSetDevice(e->device));
   // the fast mode's remainder buffers (sort ping-pong, piece ranges, segment compression): none
   // in the exact-only build -- about 10 GB per engine at C4, room for more engines in turn
   constexpr bool kFm = VN_FAST_MODE != 0;
-  // the histo path (main and replay streams) is the critical path: it gets the high queue
-  // priority, the side stream's counters / gauges / sets fill whatever CUs it leaves
-  int prio_lo = 0, prio_hi = 0;
-  VN_HIP_CHECK(hipDeviceGetStreamPriorityRange(&prio_lo, &prio_hi));
-  VN_HIP_CHECK(hipStreamCreateWithPriority(&e->st, hipStreamNonBlocking, prio_hi));
-  // Queue priority does not preempt: once the long set merge and the replay of the keys under
-  // the threshold (100k+ workgroups, some running for milliseconds) fill the CUs, the
-  // remainder rounds' chain workgroups (~100 KiB of LDS each) wait for a CU to drain -- and a
-  // workgroup waits inside the shader engine it was dealt to.  Those two streams therefore
-  // leave the last quarter of the CU mask to the main stream.  Measured on gfx950
+  // The histo path (main and replay streams) is the critical path, and a running workgroup is not
+  // preempted: once the long set merge and the replay of the keys under the threshold (100k+
+  // workgroups, some running for milliseconds) fill the CUs, the remainder rounds' chain
+  // workgroups (~100 KiB of LDS each) wait for a CU to drain -- and a workgroup waits inside the
+  // shader engine it was dealt to.  Those two streams therefore leave the last quarter of the CU
+  // mask to the main stream.  Measured on gfx950
   // (tools/probe/cumask_probe.hip): mask bit i is XCC i % 8, shader engine (i / 8) % 4, CU
   // i / 32 within it, so bits [3/4 ncu, ncu) are 2 CUs in every shader engine of every XCC.
   {
@@ -126,24 +132,32 @@ void create_impl(vn_engine* e) {
 #ifndef VN_NO_CU_MASK
 #define VN_NO_CU_MASK 0  // (build knob: every stream unmasked -- the profiling runs of DESIGN.md §8)
 #endif
-    e->prio_hi = prio_hi;
-    e->prio_lo = prio_lo;
     e->rmask = rmask;
-// The main stream CU-masked to every CU: a CU-masked stream gets a hardware queue of its own,
-// where an unmasked one shares one of the GPU_MAX_HW_QUEUES with other streams -- with several
-// engines in turn an engine's ingest front then sat in one in-order queue behind another
-// window's 170 ms chain.  Measured: C4 at N = 1, 74.2 -> 71.7 ms per window at
-// four engines, 71.4 / 72.4 at five / six (96 / 92 before); the N = 8 owner's share 45.9 ms at
-// four engines, 36.1 at six (profiles/r06_streams/).  (It gives up the high queue priority.)
+#ifndef VN_SIDE_MAIN
+#define VN_SIDE_MAIN 0  // (A/B build knob: counters, gauges and sets on the main stream, no side stream)
+#endif
+    // vn_config.replay_reserved_cus: the longest batched replays (one workgroup each, hundreds of
+    // ms, latency-bound at one wave per SIMD) on the last CUs, which every other stream of the
+    // engine leaves alone -- the other windows' sorts and scatters no longer share those CUs'
+    // SIMDs with them.  Whole groups of 8 CUs (one per XCC), at most a quarter of the chip (the
+    // quarter the replay masks above already leave to the main stream)
+    const uint32_t reserved = e->cfg.replay_reserved_cus && !VN_SIDE_MAIN && ncu >= 64
+                                  ? std::min<uint32_t>((e->cfg.replay_reserved_cus + 7u) & ~7u, ncu / 4)
+                                  : 0;
+// The main stream CU-masked to every CU (every CU but the reserved ones): a CU-masked stream
+// gets a hardware queue of its own, where an unmasked one shares one of the GPU_MAX_HW_QUEUES
+// with other streams -- with several engines in turn an engine's ingest front then sat in one
+// in-order queue behind another window's 170 ms chain.  Measured: C4 at N = 1, 74.2 -> 71.7 ms
+// per window at four engines, 71.4 / 72.4 at five / six (96 / 92 before); the N = 8 owner's
+// share 45.9 ms at four engines, 36.1 at six (profiles/r06_streams/).
 #ifndef VN_ST_FULLMASK
 #define VN_ST_FULLMASK 1
 #endif
-    if (VN_ST_FULLMASK && ncu >= 64) {
-      std::vector<uint32_t> fmask((ncu + 31) / 32, 0u);
-      for (uint32_t i = 0; i < ncu; i++) fmask[i / 32] |= 1u << (i % 32);
-      VN_HIP_CHECK(hipStreamDestroy(e->st));
-      VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&e->st, (uint32_t)fmask.size(), fmask.data()));
+    if (reserved || (VN_ST_FULLMASK && ncu >= 64)) {
+      e->amask.assign((ncu + 31) / 32, 0u);
+      for (uint32_t i = 0; i < ncu - reserved; i++) e->amask[i / 32] |= 1u << (i % 32);
     }
+    e->st = stream_on(e->amask);
     if (VN_NO_CU_MASK || ncu < 64 || hipExtStreamCreateWithCUMask(&e->st2, (uint32_t)mask.size(), mask.data()) != hipSuccess ||
         hipExtStreamCreateWithCUMask(&e->st5, (uint32_t)rmask.size(), rmask.data()) != hipSuccess) {
       (void)hipGetLastError();
@@ -152,14 +166,11 @@ void create_impl(vn_engine* e) {
           (void)hipStreamDestroy(*p);
           *p = nullptr;
         }
-      VN_HIP_CHECK(hipStreamCreateWithPriority(&e->st2, hipStreamNonBlocking, prio_lo));
-      VN_HIP_CHECK(hipStreamCreateWithPriority(&e->st5, hipStreamNonBlocking, prio_hi));
+      e->st2 = stream_on({});
+      e->st5 = stream_on({});
       e->side_cus = ncu;
       e->rmask.clear();
     }
-#ifndef VN_SIDE_MAIN
-#define VN_SIDE_MAIN 0  // (A/B build knob: counters, gauges and sets on the main stream, no side stream)
-#endif
     if (VN_SIDE_MAIN && e->st2) {
       VN_HIP_CHECK(hipStreamDestroy(e->st2));
       e->st2 = nullptr;
@@ -168,22 +179,12 @@ void create_impl(vn_engine* e) {
     VN_HIP_CHECK(hipEventCreateWithFlags(&e->ev_join5, hipEventDisableTiming));
     VN_HIP_CHECK(hipEventCreateWithFlags(&e->ev_rest5, hipEventDisableTiming));
     VN_HIP_CHECK(hipEventCreateWithFlags(&e->ev_bulk, hipEventDisableTiming));
-    // vn_config.replay_reserved_cus: the longest batched replays (one workgroup each, hundreds of
-    // ms, latency-bound at one wave per SIMD) on the last CUs, which every other stream of the
-    // engine leaves alone -- the other windows' sorts and scatters no longer share those CUs'
-    // SIMDs with them.  Whole groups of 8 CUs (one per XCC), at most a quarter of the chip (the
-    // quarter the replay masks above already leave to the main stream)
-    e->reserved_cus = 0;
-    if (e->cfg.replay_reserved_cus && e->st2 && ncu >= 64) {
-      const uint32_t r = std::min<uint32_t>((e->cfg.replay_reserved_cus + 7u) & ~7u, ncu / 4);
+    e->reserved_cus = reserved;
+    if (reserved) {
       std::vector<uint32_t> tmask((ncu + 31) / 32, 0u);
-      e->amask.assign((ncu + 31) / 32, 0u);
-      for (uint32_t i = 0; i < ncu; i++) (i >= ncu - r ? tmask : e->amask)[i / 32] |= 1u << (i % 32);
-      VN_HIP_CHECK(hipStreamDestroy(e->st));
-      VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&e->st, (uint32_t)e->amask.size(), e->amask.data()));
-      VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&e->st6, (uint32_t)tmask.size(), tmask.data()));
+      for (uint32_t i = ncu - reserved; i < ncu; i++) tmask[i / 32] |= 1u << (i % 32);
+      e->st6 = stream_on(tmask);
       VN_HIP_CHECK(hipEventCreateWithFlags(&e->ev_join6, hipEventDisableTiming));
-      e->reserved_cus = r;
     }
     // A/B build knob (make variant VARIANT_FLAGS=-DVN_EARLY_TOP=1): the longest batched replays on
     // a stream of their own, started once their own chunks are sorted (ingest_histo.hip).  Measured
@@ -195,8 +196,7 @@ void create_impl(vn_engine* e) {
 #endif
     e->early_top = VN_EARLY_TOP != 0;
     if (!e->st6 && e->early_top) {
-      if (e->side_cus != ncu) VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&e->st6, (uint32_t)rmask.size(), rmask.data()));
-      else VN_HIP_CHECK(hipStreamCreateWithPriority(&e->st6, hipStreamNonBlocking, prio_hi));
+      e->st6 = stream_on(e->rmask);  // (empty where the CU masks were refused)
       VN_HIP_CHECK(hipEventCreateWithFlags(&e->ev_join6, hipEventDisableTiming));
     }
   }
@@ -795,7 +795,7 @@ void ingest_device(vn_engine* e, const vn_batch* b) {
     side_join(e);
   } else {
     // the histo grouping sort (critical path) is queued first on the main stream; then
-    // counters, gauges and sets on the low-priority side stream (none of them waits on the
+    // counters, gauges and sets on the side stream (none of them waits on the
     // host); then the rest of the histo path, whose host round trips no longer hold back
     // the side work -- it fills the GPU while the replays and remainder rounds run
     side_begin(e);  // the side stream waits for what the main stream held before this call
@@ -907,13 +907,7 @@ void take_decode_error(vn_engine* e) {
 // st3 / st4 (the fast mode's fork) and st_ctr (the split counters' combine), at first use
 void ensure_aux_streams(vn_engine* e, bool fork, bool ctr) {
   auto make = [&](hipStream_t& s, bool replay_mask) {
-    if (s) return;
-    if (e->reserved_cus)
-      VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&s, (uint32_t)e->amask.size(), e->amask.data()));
-    else if (replay_mask && !e->rmask.empty())
-      VN_HIP_CHECK(hipExtStreamCreateWithCUMask(&s, (uint32_t)e->rmask.size(), e->rmask.data()));
-    else
-      VN_HIP_CHECK(hipStreamCreateWithPriority(&s, hipStreamNonBlocking, e->prio_hi));
+    if (!s) s = stream_on(replay_mask && !e->reserved_cus && !e->rmask.empty() ? e->rmask : e->amask);
   };
   if (fork) {
     make(e->st3, true);

@@ -1450,8 +1450,8 @@ void histo_process(vn_engine* e, uint64_t n, const HistoGroups& g, const double*
       VN_HIP_CHECK(hipStreamWaitEvent(e->st5, e->ev_fork5, 0));
       if (e->st6) VN_HIP_CHECK(hipStreamWaitEvent(e->st6, e->ev_fork5, 0));
       // (VN_BULK_SIDE: the other keys' replays -- throughput work that ends long before the
-      // chain -- on the low-priority side stream, so the next windows' ingest fronts on their
-      // high-priority main streams do not queue behind them)
+      // chain -- on the side stream, so the next windows' ingest fronts on their main streams do not
+      // queue behind them)
       const bool bulk = kBulkSide && e->st2 && e->ev_bulk;
       hipStream_t sb = s;
       if (bulk) {

@@ -111,9 +111,9 @@ vn_engine* split_engine(vn_engine* e, uint64_t records) {
   S.aux = a;
   a->long_replay = 1024;  // the owner's gathered prefixes (4096 records) are its critical path
   {
-    // a stream of its own hardware queue: the engine's high-priority streams (this engine's
-    // main and hot-prefix streams) share one, and behind their event waits the combine's short
-    // kernels would queue until this engine's replay ends
+    // an unmasked stream, so it shares no hardware queue with this engine's masked ones (main,
+    // replay, side): behind their event waits the combine's short kernels would queue until this
+    // engine's replay ends
     hipStream_t s = nullptr;
     VN_HIP_CHECK(hipStreamSynchronize(a->st));
     VN_HIP_CHECK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
