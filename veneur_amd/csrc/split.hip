@@ -101,6 +101,9 @@ vn_engine* split_engine(vn_engine* e, uint64_t records) {
   c.capacity[VN_HISTO] = kMaxSplitKeys;
   c.capacity[VN_SET] = kMaxSplitKeys;
   c.max_batch_records = std::max<uint64_t>(records, 1u << 21);
+  // (the engine's per-class caps hold its own batches; the split engine's are the gathered records
+  // of every rank, checked against max_records alone)
+  std::fill(std::begin(c.max_batch_class_records), std::end(c.max_batch_class_records), 0u);
   c.max_batch_member_bytes = 0;
   vn_engine* a = nullptr;
   if (vn_engine_create(&c, &a) != VN_OK) {
