@@ -904,10 +904,14 @@ void take_decode_error(vn_engine* e) {
     throw DecodeError("malformed import payload");
   }
 }
-// st3 / st4 (the fast mode's fork) and st_ctr (the split counters' combine), at first use
+// st3 / st4 (the fast mode's fork) and st_ctr (the split counters' combine), at first use.  Unmasked
+// where no CUs are reserved and no replays run on them: with a full CU mask, so a hardware queue of
+// its own, st_ctr's queues are four more beside four engines' twelve masked ones and every window
+// slows (bench.py --split --sim-world 8 --sim-rank 3, four engines in turn: 63.8 ms per window
+// against 56.4 unmasked).
 void ensure_aux_streams(vn_engine* e, bool fork, bool ctr) {
   auto make = [&](hipStream_t& s, bool replay_mask) {
-    if (!s) s = stream_on(replay_mask && !e->reserved_cus && !e->rmask.empty() ? e->rmask : e->amask);
+    if (!s) s = stream_on(e->reserved_cus ? e->amask : replay_mask ? e->rmask : std::vector<uint32_t>{});
   };
   if (fork) {
     make(e->st3, true);
