@@ -27,3 +27,14 @@ def test_every_stream_has_the_default_priority():
     hits = ["%s: %s" % (n, m.group(0)) for n, t in _sources("veneur_amd", "include", "tools", "tests", "bench.py",
                                                            "__graft_entry__.py") for m in bad.finditer(t)]
     assert not hits, hits
+
+
+def test_no_build_selects_the_division_that_faulted():
+    """A build whose replays divide with ddiv_nr gave wrong digests and GPU faults, cause unproven:
+    no macro selects it, and only the diagnostic entry instantiates it."""
+    src = _sources("veneur_amd", "include", ext=(".hip", ".h", ".cpp", ".py", "Makefile"))
+    assert not [n for n, t in src if re.search(r"VN_INDEX_NR|VN_NR_", t)]
+    uses = [(n, m.group(0)) for n, t in src for m in re.finditer(r"(index_estimate|asin_go_sel)<(?!false)[^>]*>", t)]
+    assert uses == [("veneur_amd/csrc/capi.hip", "index_estimate<true>"), ("veneur_amd/csrc/gomath.h", "asin_go_sel<NR>")]
+    decl = [t for n, t in src if n.endswith("gomath.h")][0]
+    assert re.findall(r"template <bool NR[^>]*>", decl) == ["template <bool NR = false>"] * 2

@@ -170,10 +170,10 @@ VN_HD double asin_go(double x) {
 // of asin's two and satan's three paths is one division feeding one xatan, so the paths
 // share that code (x / 1.0 == x exactly) and a wave no longer runs each path in turn.
 // Bit-identical to asin_go for every input in [-1, 1] (checked against the oracle).
-#ifndef VN_INDEX_NR
-#define VN_INDEX_NR false  // (build knob: true evaluates indexEstimate with ddiv_nr -- not kept)
-#endif
-template <bool NR = VN_INDEX_NR>  // NR: the divisions as ddiv_nr (indexEstimate's argument range); false: ddiv
+// NR: the divisions as ddiv_nr (indexEstimate's argument range), for vn_diag_index_estimate only.
+// The replays divide with ddiv and no build makes them do otherwise: a build with ddiv_nr at every
+// call site faulted the GPU in the batched replay, and what in it did so was not shown.
+template <bool NR = false>
 VN_HD double asin_go_sel(double x) {
   const double Morebits = 6.123233995736765886130e-17, Tan3pio8 = 2.41421356237309504880;
   const double ax = x < 0 ? -x : x;
@@ -223,7 +223,7 @@ VN_HD double from_ordered_bits(uint64_t k) {
 
 // tdigest indexEstimate (merging_digest.go:240-243): compression * (asin(2q-1)/pi + 0.5)
 // indexEstimate (merging_digest.go:240-243) for q in [0, 1]; NR as asin_go_sel
-template <bool NR = VN_INDEX_NR>
+template <bool NR = false>
 VN_HD double index_estimate(double compression, double q) {
   const double a = asin_go_sel<NR>(dsub(dmul(2.0, q), 1.0));
   return dmul(compression, dadd(NR ? ddiv_nr(a, kPi) : ddiv(a, kPi), 0.5));
