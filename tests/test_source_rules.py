@@ -38,3 +38,14 @@ def test_no_build_selects_the_division_that_faulted():
     assert uses == [("veneur_amd/csrc/capi.hip", "index_estimate<true>"), ("veneur_amd/csrc/gomath.h", "asin_go_sel<NR>")]
     decl = [t for n, t in src if n.endswith("gomath.h")][0]
     assert re.findall(r"template <bool NR[^>]*>", decl) == ["template <bool NR = false>"] * 2
+
+
+def test_tools_repeat_no_failing_case():
+    """The tools measure; they run no test's case in a loop, select no build with recorded faults
+    and read no log for a fault to go on after it.  What they run is in the tree."""
+    src = [(n, t) for n, t in _sources("tools", "bench.py") if not n.endswith((".hip", ".c"))]
+    bad = re.compile(r"from tests\.test_|import tests\.test_|libveneur_amd_nr|Memory access fault|illegal memory access|"
+                     r"\bFAILED\b")
+    assert not ["%s: %s" % (n, m.group(0)) for n, t in src for m in bad.finditer(t)]
+    named = re.compile(r"(?<![\w/.])((?:tools|tests)/[\w/]+\.(?:py|sh|hip|c))\b")
+    assert not ["%s: %s" % (n, p) for n, t in src for p in named.findall(t) if not os.path.exists(os.path.join(ROOT, p))]

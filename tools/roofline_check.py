@@ -5,7 +5,7 @@ bench.py times its kernels over its last --timing-steps steps with HIP events on
 stream, every class serialised on that stream (the earlier, timed steps run the classes
 concurrently on several streams, so their launches share the GPU and last longer).  This reads
 the trace of `rocprofv3 --kernel-trace ... -- python3 bench.py ... --timing-steps N` (the timing
-steps are the run's last steps: tools/gpu/r03_prof.sh), and for every row of the bench's
+steps are the run's last steps: the prof step of tools/gpu/run.sh), and for every row of the bench's
 roofline.kernels prints the trace's time of the same launches (the bench's launch count of that
 kernel, largest grids first) beside the bench's figure, and the roofline fraction at the trace's
 time.  With an output path it also writes the per-kernel statistics of those N steps (rocprofv3

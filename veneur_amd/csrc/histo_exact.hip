@@ -3164,10 +3164,9 @@ __device__ void replay_key_fast(const ExactCtx& x, const uint32_t k, MwSharedL& 
   };
   // the pending temps (a call's first merge of a continuing key, a final or flush-ready merge):
   // wave 0 sorts them and merges them with the one-wave merge (Go's mergeAllTemps restated), then
-  // rebuilds the main prefix.  (The four-wave fast merge out of line here, merge_step_cold, gave
-  // wrong digests in continuing calls in some builds -- tools/probe/repro_batch3_calls.py, DESIGN.md
-  // §4 -- while the same merge inlined for every chunk stayed exact: this merge, once per key and
-  // call, takes the plain path.)
+  // rebuilds the main prefix.  (The four-wave fast merge out of line here gave wrong digests in
+  // continuing calls in some builds, while the same merge inlined for every chunk stayed exact:
+  // this merge, once per key and call, takes the plain path.)
   auto merge_pend = [&]() {
     if (wv == 0) {
       const double tw_ = temp_weight(L.tw, np);
