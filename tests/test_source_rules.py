@@ -49,3 +49,17 @@ def test_tools_repeat_no_failing_case():
     assert not ["%s: %s" % (n, m.group(0)) for n, t in src for m in bad.finditer(t)]
     named = re.compile(r"(?<![\w/.])((?:tools|tests)/[\w/]+\.(?:py|sh|hip|c))\b")
     assert not ["%s: %s" % (n, p) for n, t in src for p in named.findall(t) if not os.path.exists(os.path.join(ROOT, p))]
+
+
+def test_device_code_is_built_without_packed_fp32():
+    """Some forms of the packed FP32 instructions, which the compiler makes from ordinary float
+    code, have given wrong results now and then: every HIP compile line turns them off."""
+    flag = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+    (_, mk), = _sources("veneur_amd/Makefile")
+    assert "NO_PACKED_FP32 := " + flag in mk
+    lines = [ln for ln in mk.splitlines() if "$(HIPCC)" in ln and " -c " in ln]
+    assert lines and all("$(CXXFLAGS)" in ln for ln in lines)
+    assert re.search(r"^CXXFLAGS \?= (.*\\\n)*.*\$\(NO_PACKED_FP32\)", mk, re.M)
+    hip = _sources("veneur_amd", "tools", "include", ext=(".hip", ".h"))
+    assert not [n for n, t in hip for ln in t.splitlines() if "Build: hipcc" in ln and flag not in ln]
+    assert not [n for n, t in hip if re.search(r"v_pk_(add|mul|fma)_f32", t)]

@@ -1,5 +1,5 @@
 // Host cost of hipLaunchKernel on MI355X while other streams hold long-running kernels.
-// Build: hipcc -O2 --offload-arch=gfx950 launch_probe.hip -o launch_probe
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops launch_probe.hip -o launch_probe
 // Cases: idle device; a long kernel on a second stream; the same on a CU-masked stream;
 // small (16 B) vs large (512 B) kernel arguments; launches into a captured hipGraph.
 #include <hip/hip_runtime.h>

@@ -1,5 +1,5 @@
 // Single-wave latency calibration for the exact t-digest replay (gfx950).
-// Build: hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -I../../veneur_amd/csrc ubench.hip -o ubench
+// Build: hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -I../../veneur_amd/csrc ubench.hip -o ubench
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include "gomath.h"
